@@ -59,10 +59,11 @@ template <> struct q8_scale<false> {
         least = __uint_as_float(0x3f800000u | (a & 0x7fffffu));
         inv = 1.0f / least;
     }
-    // the quotient correctly rounded: one correction with what the product by the rounded reciprocal leaves over
+    // The quotient rounded once: x * 448 is t + lo (it has up to 27 digits), and y is corrected by what it leaves over of both; the second rounding differs from the quotient's own only where that is
+    // within 2^-23 of a step of the middle between two floats.  Without lo one in four quotients beside a border of e4m3 came out a step of 32 bits off, one in twenty on the border's other side
     __device__ __forceinline__ float of(float x) const {
-        const float t = x * to, y = t * inv;
-        return __builtin_fmaf(__builtin_fmaf(-y, least, t), inv, y);
+        const float t = x * to, lo = __builtin_fmaf(x, to, -t), y = t * inv;
+        return __builtin_fmaf(__builtin_fmaf(-y, least, t) + lo, inv, y);
     }
 };
 
