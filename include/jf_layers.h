@@ -545,7 +545,8 @@ JL_API int jl_moe_gemm_gated(const void *X, const void *Wt, int dtype, int32_t K
  * e4m3 values (OCP: largest 448, no infinities) in rows padded with zeros to whole blocks of 128 columns, with a scale for each row and block (activations) or for each block of 128 x 128
  * (weights).  Scales are bytes (JL_SCALE_E8M0: 2^(byte - 127), the least power of two that leaves the block within 448, 2^-126 at least) or floats (JL_SCALE_F32: the block's largest
  * magnitude over 448, 2^-126 at least).  A block with an infinity or a NaN is all NaN, its scale too.
- * Rows have up to 2^30 columns.  Activations' scales lie block by block: scale[b * s_ld + n], s_ld >= N; weights' row of blocks by row of blocks: scale[rb * s_ld + b].  q at 8-byte borders (16 where a product reads it). */
+ * Rows have up to 2^30 columns; a launch takes fewer than 2^32 threads, more are refused: 64 for 512 columns of a row (norms: 64 a row up to 1024 columns, 256 up to 8192, 1024 beyond), in products
+ * 256 or 512 for a tile, and 512 for 16 rows of w where x has one or two (fewer than 2^27 rows of w).  Activations' scales lie block by block: scale[b * s_ld + n], s_ld >= N; weights' row of blocks by row of blocks: scale[rb * s_ld + b].  q at 8-byte borders (16 where a product reads it). */
 #define JL_SCALE_E8M0 0
 #define JL_SCALE_F32 1
 /* rows of x [N, W], float or bfloat16 (`dtype`), ld apart */

@@ -14,6 +14,9 @@ constexpr int Q8_BLOCK = 128;
 constexpr int Q8_MAX_COLS = 1 << 30;                                // columns stay within 32 bits with what a wavefront takes beyond them
 constexpr uint32_t Q8_LEAST = 0x04e00000u;                          // 448 * 2^-126: a block of smaller values is scaled as if this were its largest
 
+// whether workgroups of so many threads are more than a launch takes: fewer than 2^32 threads altogether
+static inline bool q8_too_many(int64_t workgroups, int threads) { return workgroups > (int64_t)UINT32_MAX / threads; }
+
 // the largest of |bits| over the 16 lanes of a row of the wavefront, in every one of them
 __device__ __forceinline__ uint32_t q8_max16(uint32_t v) {
 #define Q8_STEP(ctrl) { const uint32_t o = (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, ctrl, 0xF, 0xF, true); v = v > o ? v : o; }

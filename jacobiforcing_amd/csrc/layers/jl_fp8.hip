@@ -39,7 +39,7 @@ template <bool UNIT>
 static int fp8_rows_launch(const char *what, const void *x, int dtype, int64_t N, int64_t ld, int W, const Q8Unit &unit, const Q8Out &out, int scale_type, hipStream_t st) {
     const int chunks = (W + 511) / 512;
     const int64_t blocks = (N * chunks + 3) / 4;
-    if (N > INT32_MAX || blocks > INT32_MAX) return jl_fail(JL_E_INVALID, "%s: more rows than a launch takes", what);
+    if (N > INT32_MAX || q8_too_many(blocks, 256)) return jl_fail(JL_E_INVALID, "%s: more rows than a launch takes", what);
     JL_DISPATCH(dtype, {
         auto go = [&](auto kern) { kern<<<(unsigned)blocks, 256, 0, st>>>((const T *)x, ld, N, W, chunks, unit, out); };
         constexpr int U = sizeof(T) == 2 ? 8 : 4;
@@ -150,8 +150,14 @@ __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void fp8_norm_kernel(T *__
         }
 }
 
-template <typename T, bool E8, int U, bool WHOLE> static void fp8_norm_launch(T *x, const Q8Norm &a, const Q8Out &out, hipStream_t st) {
-    auto go = [&](auto kern, int waves) { kern<<<(unsigned)(waves == 1 ? (a.N + 3) / 4 : a.N), waves == 1 ? 256 : 64 * waves, 0, st>>>(x, a, out); };
+template <typename T, bool E8, int U, bool WHOLE> static int fp8_norm_launch(T *x, const Q8Norm &a, const Q8Out &out, hipStream_t st) {
+    int rc = JL_OK;
+    auto go = [&](auto kern, int waves) {
+        const int64_t blocks = waves == 1 ? (a.N + 3) / 4 : a.N;
+        const int threads = waves == 1 ? 256 : 64 * waves;
+        if (a.N > INT32_MAX || q8_too_many(blocks, threads)) rc = jl_fail(JL_E_INVALID, "jl_add_rmsnorm_fp8: more rows than a launch takes");
+        else kern<<<(unsigned)blocks, threads, 0, st>>>(x, a, out);
+    };
     const int chunks = (a.W + 511) / 512;
     if (chunks <= 1) go(fp8_norm_kernel<T, E8, U, WHOLE, 1, 1>, 1);
     else if (chunks <= 2) go(fp8_norm_kernel<T, E8, U, WHOLE, 1, 2>, 1);
@@ -160,6 +166,7 @@ template <typename T, bool E8, int U, bool WHOLE> static void fp8_norm_launch(T 
     else if (chunks <= 16) go(fp8_norm_kernel<T, E8, U, WHOLE, 4, 4>, 4);
     else if (chunks <= 64) go(fp8_norm_kernel<T, E8, U, WHOLE, 16, 4>, 16);
     else go(fp8_norm_kernel<T, E8, U, WHOLE, 16, 0>, 16);
+    return rc != JL_OK ? rc : jl_check_launch("fp8_norm_kernel");
 }
 
 extern "C" int jl_add_rmsnorm_fp8(void *x, int dtype, int64_t x_ld, const void *y, int y_dtype, int64_t y_ld, const void *w, int w_dtype, float eps, int64_t N, int32_t W, uint8_t *q, int64_t q_ld,
@@ -169,20 +176,18 @@ extern "C" int jl_add_rmsnorm_fp8(void *x, int dtype, int64_t x_ld, const void *
     if (!x || x_ld < W || (y && y_ld < W) || !known(dtype) || !known(y_dtype) || !known(w_dtype)) return jl_fail(JL_E_INVALID, "jl_add_rmsnorm_fp8: null pointer, bad sizes or types");
     const Q8Out out = {q, q_ld, scale, s_ld};
     if (const int bad = q8_out_bad("jl_add_rmsnorm_fp8", out, N, W, scale_type)) return bad;
-    if (N > INT32_MAX) return jl_fail(JL_E_INVALID, "jl_add_rmsnorm_fp8: more rows than a launch takes");
     const Q8Norm a = {x_ld, y, y_dtype, y_ld, w, w_dtype, eps, N, W};
     const bool floats = dtype == JL_F32 || (y && y_dtype == JL_F32);      // loads of four values, or of eight
     JL_DISPATCH(dtype, {
         auto go = [&](auto e8, auto whole) {
-            if (floats) fp8_norm_launch<T, decltype(e8)::value, 4, decltype(whole)::value>((T *)x, a, out, (hipStream_t)stream);
-            else fp8_norm_launch<T, decltype(e8)::value, 8, decltype(whole)::value>((T *)x, a, out, (hipStream_t)stream);
+            if (floats) return fp8_norm_launch<T, decltype(e8)::value, 4, decltype(whole)::value>((T *)x, a, out, (hipStream_t)stream);
+            return fp8_norm_launch<T, decltype(e8)::value, 8, decltype(whole)::value>((T *)x, a, out, (hipStream_t)stream);
         };
         const std::true_type yes;
         const std::false_type no;
-        if (scale_type == JL_SCALE_E8M0) { if (W % 8 == 0) go(yes, yes); else go(yes, no); }
-        else { if (W % 8 == 0) go(no, yes); else go(no, no); }
+        if (scale_type == JL_SCALE_E8M0) return W % 8 == 0 ? go(yes, yes) : go(yes, no);
+        return W % 8 == 0 ? go(no, yes) : go(no, no);
     });
-    return jl_check_launch("fp8_norm_kernel");
 }
 
 // ---- weights: a scale for each block of 128 x 128, a workgroup's -----------------------------------------------------------------------------------------

@@ -537,14 +537,14 @@ template <bool E8, bool GATED, int TM, int TN, int WM, int WN, int RING>
 static int fp8_tile_launch(const Fp8Product &a, const Fp8Result &r, const Q8Out &out, const Fp8Unit &unit, int splits, float *parts, hipStream_t st) {
     constexpr int lds = RING * (TM + TN) * Q8_BLOCK;
     auto kern = fp8_tile_kernel<E8, GATED, TM, TN, WM, WN, RING>;
+    const int64_t row_tiles = (a.N + TM - 1) / TM, tiles = row_tiles * (((int64_t)a.O + TN - 1) / TN);
+    const int64_t items = (tiles * splits + 7) / 8 * 8, blocks = TM == 256 && E8 && items > 256 ? 256 : items;      // (256 CUs)
+    if (tiles * splits > INT32_MAX / 2 || q8_too_many(blocks, 64 * WM * WN)) return jl_fail(JL_E_INVALID, "fp8_tile_kernel: more tiles than a launch takes");
     if (lds > 48 * 1024) {                                          // with the scales beside them beyond 64 KB
         const hipError_t e = hipFuncSetAttribute((const void *)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
         if (e != hipSuccess) return jl_fail(JL_E_LAUNCH, "fp8_tile_kernel: cannot get %d bytes of LDS: %s", lds, hipGetErrorString(e));
     }
-    const int64_t row_tiles = (a.N + TM - 1) / TM, tiles = row_tiles * ((a.O + TN - 1) / TN);
-    if (tiles * splits > INT32_MAX / 2) return jl_fail(JL_E_INVALID, "fp8_tile_kernel: more tiles than a launch takes");
-    const int64_t items = (tiles * splits + 7) / 8 * 8;
-    kern<<<(unsigned)(TM == 256 && E8 && items > 256 ? 256 : items), 64 * WM * WN, lds, st>>>(a, r, out, unit, Fp8Tiles{(int)row_tiles, (int)tiles, splits, parts});      // (256 CUs)
+    kern<<<(unsigned)blocks, 64 * WM * WN, lds, st>>>(a, r, out, unit, Fp8Tiles{(int)row_tiles, (int)tiles, splits, parts});
     return jl_check_launch("fp8_tile_kernel");
 }
 
@@ -643,10 +643,14 @@ extern "C" int jl_linear_fp8(const jl_fp8_product *p, const void *bias, int bias
     case F8_64x128_MANY: rc = F8_TILE(64, 128, 1, 4, 3); break;
     case F8_256x256: rc = F8_TILE(256, 256, 2, 4, 2); break;
     default: {
-        auto go = [&](auto kern, int nt, int ot, int nw) { kern<<<dim3((unsigned)((p->O + 16 * ot - 1) / (16 * ot)), (unsigned)((p->N + 16 * nt - 1) / (16 * nt))), 64 * nw, 0, st>>>(a, r); };
-        if (e8) { if (p->N <= 16) go(fp8_few_kernel<true, 1, 1, 8, 4>, 1, 1, 8); else go(fp8_few_kernel<true, 4, 2, 4, 1>, 4, 2, 4); }
-        else { if (p->N <= 16) go(fp8_few_kernel<false, 1, 1, 8, 4>, 1, 1, 8); else go(fp8_few_kernel<false, 4, 2, 4, 1>, 4, 2, 4); }
-        return jl_check_launch("fp8_few_kernel");
+        auto go = [&](auto kern, int nt, int ot, int nw) {
+            const int64_t cols = (p->O + 16 * (int64_t)ot - 1) / (16 * ot);
+            if (q8_too_many(cols, 64 * nw)) return jl_fail(JL_E_INVALID, "jl_linear_fp8: more rows of w than a launch takes");
+            kern<<<dim3((unsigned)cols, (unsigned)((p->N + 16 * nt - 1) / (16 * nt))), 64 * nw, 0, st>>>(a, r);
+            return jl_check_launch("fp8_few_kernel");
+        };
+        if (e8) return p->N <= 16 ? go(fp8_few_kernel<true, 1, 1, 8, 4>, 1, 1, 8) : go(fp8_few_kernel<true, 4, 2, 4, 1>, 4, 2, 4);
+        return p->N <= 16 ? go(fp8_few_kernel<false, 1, 1, 8, 4>, 1, 1, 8) : go(fp8_few_kernel<false, 4, 2, 4, 1>, 4, 2, 4);
     }
     }
 #undef F8_TILE
@@ -675,8 +679,11 @@ extern "C" int jl_linear_gated_fp8(const jl_fp8_product *p, int32_t kind, float 
     case F8_256x256: return F8_TILE(256, 256, 2, 4, 2);
     }
 #undef F8_TILE
-    auto go = [&](auto kern, int nt) { kern<<<dim3((unsigned)(F / Q8_BLOCK), (unsigned)((p->N + 16 * nt - 1) / (16 * nt))), 1024, 0, st>>>(a, F, kind, limit, alpha, shift, out); };
-    if (e8) { if (p->N <= 16) go(fp8_few_gated_kernel<true, 1, 4>, 1); else go(fp8_few_gated_kernel<true, 4, 1>, 4); }
-    else { if (p->N <= 16) go(fp8_few_gated_kernel<false, 1, 4>, 1); else go(fp8_few_gated_kernel<false, 4, 1>, 4); }
-    return jl_check_launch("fp8_few_gated_kernel");
+    auto go = [&](auto kern, int nt) {
+        if (q8_too_many(F / Q8_BLOCK, 1024)) return jl_fail(JL_E_INVALID, "jl_linear_gated_fp8: more rows of w than a launch takes");
+        kern<<<dim3((unsigned)(F / Q8_BLOCK), (unsigned)((p->N + 16 * nt - 1) / (16 * nt))), 1024, 0, st>>>(a, F, kind, limit, alpha, shift, out);
+        return jl_check_launch("fp8_few_gated_kernel");
+    };
+    if (e8) return p->N <= 16 ? go(fp8_few_gated_kernel<true, 1, 4>, 1) : go(fp8_few_gated_kernel<true, 4, 1>, 4);
+    return p->N <= 16 ? go(fp8_few_gated_kernel<false, 1, 4>, 1) : go(fp8_few_gated_kernel<false, 4, 1>, 4);
 }
