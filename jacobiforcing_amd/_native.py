@@ -474,7 +474,7 @@ class _NoHost:
 
 
 def host(*rules):
-    """The host's side of the small launches (csrc/layers/jl_host.cpp), bound to the kernel libraries; built when there is none for this torch.  ``rules``: the numbers that ``linear``'s rules go by.
+    """The host's side of the small launches (csrc/layers/jl_host.cpp), bound to the kernel libraries (that of the 8-bit rows: ``host_fp8``); built when there is none for this torch.  ``rules``: the numbers that ``linear``'s rules go by.
     Where it can be neither built nor loaded the wrappers make the same launches by themselves, some us later each, and a warning says so."""
     import importlib.machinery
     import importlib.util
@@ -492,12 +492,25 @@ def host(*rules):
         return _NoHost()
     if module.version != JL_VERSION:
         raise NativeLibraryError(f"{lib} has version {module.version}, this package calls version {JL_VERSION}: build it again (python -c 'import __graft_entry__ as g; g.build()')")
-    L, address = layers(), lambda fn: C.cast(fn, C.c_void_p).value
-    symbols = {name: address(getattr(L, name)) for name in module.symbols()}
-    symbols["jl_last_error"], symbols["jl_last_error of the recurrences"], symbols["jl_last_error of the 8-bit rows"] = (
-        address(L._library(name).jl_last_error) for name in ("jl_linear_small", "jl_linear_scan", "jl_linear_fp8"))
+    L = layers()
+    symbols = {name: _address(getattr(L, name)) for name in module.symbols()}
+    symbols["jl_last_error"], symbols["jl_last_error of the recurrences"] = (_address(L._library(name).jl_last_error) for name in ("jl_linear_small", "jl_linear_scan"))
     module.bind(symbols, *rules)
     return module
+
+
+def host_fp8(module):
+    """``host()``'s module bound to the library of the 8-bit rows too, which is loaded (or built) here: at the first call that needs it."""
+    if not isinstance(module, _NoHost):
+        L = layers()
+        symbols = {name: _address(getattr(L, name)) for name in module.symbols_fp8()}
+        symbols["jl_last_error"] = _address(L._library("jl_linear_fp8").jl_last_error)
+        module.bind_fp8(symbols)
+    return module
+
+
+def _address(fn) -> int:
+    return C.cast(fn, C.c_void_p).value
 
 
 def check_layers(rc: int, what: str = ""):

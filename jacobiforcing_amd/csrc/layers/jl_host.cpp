@@ -29,10 +29,12 @@ namespace {
 #define JL_HOST_CALLS(X)                                                                                                                              \
     X(jl_linear_small) X(jl_linear_mid_ok) X(jl_linear_mid) X(jl_linear_split_ok) X(jl_linear_split) X(jl_embed_scale) X(jl_add_rmsnorm) X(jl_sandwich_norm) X(jl_output_norm) X(jl_gated_norm) \
     X(jl_gated_act) X(jl_heads_gate) X(jl_latent_prep) X(jl_latent_q_pack) X(jl_token_shift) X(jl_depth_mix_norm) X(jl_short_conv) X(jl_linear_scan) X(jl_latent_heads_run) \
-    X(jl_moe_router_blocks) X(jl_moe_router_run) X(jl_linear_mid_gated) X(jl_rms_norm) X(jl_linear_after_ok) X(jl_linear_after_run) X(jl_moe_few_ok) X(jl_moe_few_run) X(jl_moe_gemm) X(jl_moe_gemm_gated) X(jl_qk_norm_append) \
-    X(jl_quantize_fp8) X(jl_add_rmsnorm_fp8) X(jl_gated_act_fp8) X(jl_linear_fp8_floats) X(jl_linear_fp8) X(jl_linear_gated_fp8)
+    X(jl_moe_router_blocks) X(jl_moe_router_run) X(jl_linear_mid_gated) X(jl_rms_norm) X(jl_linear_after_ok) X(jl_linear_after_run) X(jl_moe_few_ok) X(jl_moe_few_run) X(jl_moe_gemm) X(jl_moe_gemm_gated) X(jl_qk_norm_append)
+// in a library of their own, which is loaded (or compiled) at the first of these calls
+#define JL_HOST_FP8_CALLS(X) X(jl_quantize_fp8) X(jl_add_rmsnorm_fp8) X(jl_gated_act_fp8) X(jl_linear_fp8_floats) X(jl_linear_fp8) X(jl_linear_gated_fp8)
 #define DECLARE(name) decltype(&name) p_##name;
 JL_HOST_CALLS(DECLARE)
+JL_HOST_FP8_CALLS(DECLARE)
 #undef DECLARE
 
 using at::Tensor;
@@ -865,6 +867,7 @@ END_CALL
 
 // ---- 8-bit rows (jl_fp8.hip, jl_fp8_linear.hip) -------------------------------------------------------------------------------------------------------------
 constexpr int64_t FP8_BLOCK = 128;
+#define CALL8(name, count) CALL(name, count) NEED(p_last_error_fp8);      // (bound last)
 // a float type or bfloat16, rows of consecutive values on the current device, no gradient wanted
 bool fp8_here(const Tensor &t) {
     return t.device().index() == c10::hip::current_device() && !(c10::GradMode::is_enabled() && t.requires_grad()) && !t._fw_grad(0).defined();
@@ -895,7 +898,7 @@ PyObject *pair(const Rows8 &r) {
 #define OUT8(r) r.q(), r.data.size(1), r.scale.data_ptr(), r.scale.stride(1)
 
 // x, type of the scales
-CALL(quantize_fp8, 2)
+CALL8(quantize_fp8, 2)
     const Tensor *x;
     at::ScalarType type;
     NEED(take(arg[0], x) && take_scales(arg[1], type) && known(*x) && fp8_matrix(*x));
@@ -907,7 +910,7 @@ CALL(quantize_fp8, 2)
 END_CALL
 
 // x, y, w, eps, type of the scales
-CALL(add_rmsnorm_fp8, 5)
+CALL8(add_rmsnorm_fp8, 5)
     const Tensor *x, *y, *w;
     double eps;
     at::ScalarType type;
@@ -926,7 +929,7 @@ CALL(add_rmsnorm_fp8, 5)
 END_CALL
 
 // z, g_col, u_col, F, kind, limit, alpha, shift, type of the scales
-CALL(gated_act_fp8, 9)
+CALL8(gated_act_fp8, 9)
     const Tensor *z;
     int32_t g_col, u_col, F, kind;
     double limit, alpha, shift;
@@ -957,7 +960,7 @@ bool fp8_operands(PyObject *const *arg, const Tensor *&x, jl_fp8_product &p) {
     return true;
 }
 // x, its scales, w, its scales, bias, type of the result
-CALL(linear_fp8, 6)
+CALL8(linear_fp8, 6)
     const Tensor *x, *bias;
     jl_fp8_product p;
     at::ScalarType type;
@@ -973,7 +976,7 @@ CALL(linear_fp8, 6)
 END_CALL
 
 // x, its scales, w, its scales, kind, limit, alpha, shift
-CALL(linear_gated_fp8, 8)
+CALL8(linear_gated_fp8, 8)
     const Tensor *x;
     jl_fp8_product p;
     int32_t kind;
@@ -986,12 +989,6 @@ CALL(linear_gated_fp8, 8)
     return pair(r);
 END_CALL
 
-// {symbol: address}, LINEAR_SMALL_ROWS, LINEAR_ONE_TILE, LINEAR_X_BYTES
-PyObject *bind(PyObject *, PyObject *args) {
-    PyObject *symbols;
-    long long rows_, tile, bytes;
-    if (!PyArg_ParseTuple(args, "O!LLL", &PyDict_Type, &symbols, &rows_, &tile, &bytes)) return nullptr;
-    small_rows = rows_; one_tile = tile; x_bytes = bytes;
 #define BIND(name)                                                                                                         \
     {                                                                                                                      \
         PyObject *v = PyDict_GetItemString(symbols, #name);                                                                \
@@ -999,26 +996,39 @@ PyObject *bind(PyObject *, PyObject *args) {
         if (!p) { if (!PyErr_Occurred()) PyErr_SetString(PyExc_KeyError, #name); return nullptr; }                         \
         p_##name = (decltype(p_##name))p;                                                                                  \
     }
+// {symbol: address}, LINEAR_SMALL_ROWS, LINEAR_ONE_TILE, LINEAR_X_BYTES
+PyObject *bind(PyObject *, PyObject *args) {
+    PyObject *symbols;
+    long long rows_, tile, bytes;
+    if (!PyArg_ParseTuple(args, "O!LLL", &PyDict_Type, &symbols, &rows_, &tile, &bytes)) return nullptr;
+    small_rows = rows_; one_tile = tile; x_bytes = bytes;
     JL_HOST_CALLS(BIND)
-#undef BIND
-    PyObject *e = PyDict_GetItemString(symbols, "jl_last_error"), *q = PyDict_GetItemString(symbols, "jl_last_error of the recurrences"), *f = PyDict_GetItemString(symbols, "jl_last_error of the 8-bit rows");
+    PyObject *e = PyDict_GetItemString(symbols, "jl_last_error"), *q = PyDict_GetItemString(symbols, "jl_last_error of the recurrences");
     if (!e || !q) { PyErr_SetString(PyExc_KeyError, "jl_last_error"); return nullptr; }
     p_last_error = (decltype(p_last_error))PyLong_AsVoidPtr(e);
     p_last_error_seq = (decltype(p_last_error))PyLong_AsVoidPtr(q);
-    p_last_error_fp8 = f ? (decltype(p_last_error))PyLong_AsVoidPtr(f) : p_last_error;
     if (PyErr_Occurred()) return nullptr;
     Py_RETURN_NONE;
 }
+// {symbol: address} of the 8-bit rows; until then their calls are not taken
+PyObject *bind_fp8(PyObject *, PyObject *args) {
+    PyObject *symbols;
+    if (!PyArg_ParseTuple(args, "O!", &PyDict_Type, &symbols)) return nullptr;
+    JL_HOST_FP8_CALLS(BIND)
+    PyObject *e = PyDict_GetItemString(symbols, "jl_last_error");
+    if (!e) { PyErr_SetString(PyExc_KeyError, "jl_last_error"); return nullptr; }
+    p_last_error_fp8 = (decltype(p_last_error))PyLong_AsVoidPtr(e);
+    if (PyErr_Occurred()) { p_last_error_fp8 = nullptr; return nullptr; }
+    Py_RETURN_NONE;
+}
+#undef BIND
 // n, k, o, bytes of an element, whether x and w are float: which of the package's products linear takes (0: the library's, 1 small, 2 split, 3 mid)
 PyObject *linear_rule(PyObject *, PyObject *args) {
     long long n, k, o, item;
     if (!PyArg_ParseTuple(args, "LLLL", &n, &k, &o, &item)) return nullptr;
     return PyLong_FromLong(rule_small(n, k, o, item) ? 1 : item == 4 ? (p_jl_linear_split_ok(n, k, o) ? 2 : 0) : p_jl_linear_mid_ok(n, k, o) ? 3 : 0);
 }
-PyObject *symbols(PyObject *, PyObject *) {
-#define NAME(name) #name,
-    static const char *const names[] = {JL_HOST_CALLS(NAME)};
-#undef NAME
+PyObject *names_list(std::initializer_list<const char *> names) {
     PyObject *list = PyList_New(0);
     for (const char *s : names) {
         PyObject *v = list ? PyUnicode_FromString(s) : nullptr;
@@ -1027,12 +1037,16 @@ PyObject *symbols(PyObject *, PyObject *) {
     }
     return list;
 }
+#define NAME(name) #name,
+PyObject *symbols(PyObject *, PyObject *) { return names_list({JL_HOST_CALLS(NAME)}); }
+PyObject *symbols_fp8(PyObject *, PyObject *) { return names_list({JL_HOST_FP8_CALLS(NAME)}); }
+#undef NAME
 
 #define FAST(name) {#name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FAST(linear), FAST(linear_add), FAST(linear_gated), FAST(rms_norm), FAST(norm_linear), FAST(act_linear), FAST(gated_norm_linear), FAST(add_rmsnorm), FAST(sandwich_norm), FAST(output_norm), FAST(gated_norm), FAST(gated_act), FAST(heads_gate), FAST(latent_prep), FAST(latent_q_pack), FAST(latent_heads),
                          FAST(token_shift), FAST(depth_mix_norm), FAST(short_conv), FAST(linear_scan), FAST(embed_scale), FAST(moe_experts), FAST(attention_args), FAST(qk_norm_append), FAST(step_tables), FAST(step_views), FAST(tile_records),
                          FAST(quantize_fp8), FAST(add_rmsnorm_fp8), FAST(gated_act_fp8), FAST(linear_fp8), FAST(linear_gated_fp8), {"bind", bind, METH_VARARGS, nullptr},
-                         {"linear_rule", linear_rule, METH_VARARGS, nullptr}, {"symbols", symbols, METH_NOARGS, nullptr}, {nullptr, nullptr, 0, nullptr}};
+                         {"linear_rule", linear_rule, METH_VARARGS, nullptr}, {"symbols", symbols, METH_NOARGS, nullptr}, {"bind_fp8", bind_fp8, METH_VARARGS, nullptr}, {"symbols_fp8", symbols_fp8, METH_NOARGS, nullptr}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_jl_host", nullptr, -1, methods};
 
 }  // namespace

@@ -1262,9 +1262,18 @@ def _no_gradient(what: str, *tensors: Optional[torch.Tensor]) -> None:
           f"{what} has no gradient: call it where none is wanted")
 
 
+_H8 = None                                           # the host side that the library of the 8-bit rows is bound to
+
+
 def _fp8_native(name: str, *args):
     """The call's native host side, or NotImplemented."""
-    return NotImplemented if is_dynamo_compiling() else getattr(_H or _host(), name)(*args)
+    global _H8
+    if is_dynamo_compiling():
+        return NotImplemented
+    h = _H or _host()
+    if _H8 is not h:
+        _H8 = N.host_fp8(h)
+    return getattr(h, name)(*args)
 
 
 def quantize_fp8(x: torch.Tensor, scale_dtype: torch.dtype = torch.float8_e8m0fnu) -> Fp8Rows:
