@@ -22,12 +22,12 @@ _FIELDS = [
     ("kv_cache_layout", str, "contiguous"),
     # "auto": bfloat16 on the GPU (float32 on the CPU); "bfloat16" / "float32" force it.  float32 = every product in true 32-bit
     ("dtype", str, "auto"),
-    # None, or "fp8": the layers' products of a Qwen2 model on 8-bit weights and rows (bfloat16 on the GPU; embedding and head stay as they are)
-    ("quantization", Optional[str], None),
     # Jacobi defaults of the engine (requests override them through SamplingParams)
     ("jacobi_enabled", bool, True), ("jacobi_block_len", int, 64), ("jacobi_max_blocks", int, 2),
     ("jacobi_spawn_ratio", float, 0.8), ("jacobi_lookahead_start_ratio", float, 0.0),
     ("jacobi_n_gram_pool_size", int, 4), ("jacobi_max_iterations", int, 128),
+    # None, or "fp8": the layers' products of a Qwen2 model on 8-bit weights and rows (bfloat16 on the GPU; embedding and head stay as they are)
+    ("quantization", Optional[str], None),
 ]
 
 
