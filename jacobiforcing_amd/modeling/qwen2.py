@@ -73,6 +73,13 @@ class Qwen2Config:
                    pad_token_id=d.get("pad_token_id") or 151643)
 
 
+def _whole_values(tensors) -> None:
+    """Refuses checkpoints whose matrices are 8-bit values beside scales: without those they would be other weights."""
+    short = [k for k, t in tensors.items() if t.is_floating_point() and t.element_size() < 2]
+    if short:
+        raise ValueError(f"{short[0]} and {len(short) - 1} more are {tensors[short[0]].dtype}: checkpoints of 8-bit values and scales are not read (16- or 32-bit ones are, and quantize_fp8 makes 8 bits of them)")
+
+
 class Qwen2Weights:
     """Flat weight container (fused QKV and gate/up so each layer is 4 GEMMs)."""
 
@@ -100,6 +107,7 @@ class Qwen2Weights:
 
     def load_state_dict(self, sd, cfg: Qwen2Config) -> None:
         """Adopt the tensors of a HF ``Qwen2ForCausalLM.state_dict()`` (fuses q/k/v and gate/up; casts to this dtype)."""
+        _whole_values(sd)
         dev, dt = self.embed.device, self.embed.dtype
         get = lambda k: sd[k].detach().to(device=dev, dtype=dt)
         self.fp8 = False
@@ -127,6 +135,7 @@ class Qwen2Weights:
             with safe_open(str(f), "pt", "cpu") as sf:
                 for k in sf.keys():
                     tensors[k] = sf.get_tensor(k)
+        _whole_values(tensors)
         dev, dt = self.embed.device, self.embed.dtype
         get = lambda k: tensors[k].to(device=dev, dtype=dt)
         self.fp8 = False
