@@ -17,7 +17,7 @@ extern "C" {
 #endif
 
 #define JL_API __attribute__((visibility("default")))
-#define JL_VERSION 146
+#define JL_VERSION 147
 #define JL_OK 0
 #define JL_E_INVALID (-1)
 #define JL_E_LAUNCH (-3)
@@ -567,6 +567,9 @@ typedef struct {
     int64_t N, x_ld, x_scale_ld, w_ld, w_scale_ld;
     int32_t K, O, scale_type;
 } jl_fp8_product;
+/* How jl_linear_fp8 (gated: jl_linear_gated_fp8) cuts a product, for tests and profiles: rows of x by rows of w in a tile ("two", "many": so many workgroups per CU; "rows": no tiles, straight from memory),
+ * and into how many shares of the depth (null: not asked for).  Which it is may change; every cut gives the same sums up to their order. */
+JL_API const char *jl_fp8_cut(const jl_fp8_product *p, int gated, int32_t *shares);
 /* out [N, O] (float or bfloat16) = x w^T (+ bias [O], null: none, of its own type), float sums rounded once; scratch of jl_linear_fp8_floats floats at a 16-byte border (0: null) */
 JL_API int64_t jl_linear_fp8_floats(const jl_fp8_product *p);
 JL_API int jl_linear_fp8(const jl_fp8_product *p, const void *bias, int bias_dtype, void *out, int64_t out_ld, int out_dtype, float *scratch, void *stream);

@@ -232,7 +232,7 @@ def raise_state_error(code: int, what: str, aux: int = 0):
 # ---- libjf_layers.so (include/jf_layers.h): layer kernels of the models whose forward is not stock PyTorch ----------------------------
 JL_F32, JL_BF16 = 0, 1
 JL_SCALE_E8M0, JL_SCALE_F32 = 0, 1
-JL_VERSION = 146                 # include/jf_layers.h: a library of another version is not called (its signatures may differ)
+JL_VERSION = 147                 # include/jf_layers.h: a library of another version is not called (its signatures may differ)
 JL_OUT_SAME, JL_OUT_F32 = 0, 2
 JL_ACT_GELU_TANH, JL_ACT_CLAMPED_SWISH, JL_ACT_SILU, JL_ACT_GELU_ERF, JL_ACT_SIGMOID, JL_ACT_NONE = 0, 1, 2, 3, 4, -1
 JL_ROUTE_SIGMOID, JL_ROUTE_SOFTMAX_RENORM, JL_ROUTE_TOP_SOFTMAX = 0, 1, 2
@@ -394,6 +394,7 @@ _LAYER_SIGNATURES = {
     "jl_add_rmsnorm_fp8": (C.c_int, [_vp, C.c_int, _i64, _vp, C.c_int, _i64, _vp, C.c_int, _f32, _i64, _i32, _vp, _i64, _vp, _i64, C.c_int, _vp]),
     "jl_gated_act_fp8": (C.c_int, [_vp, C.c_int, _i64, _i64, _i32, _i32, _i32, _i32, _f32, _f32, _f32, _vp, _i64, _vp, _i64, C.c_int, _vp]),
     "jl_quantize_weight_fp8": (C.c_int, [_vp, C.c_int, _i64, _i64, _i32, _vp, _i64, _vp, _i64, C.c_int, _vp]),
+    "jl_fp8_cut": (C.c_char_p, [C.POINTER(Fp8Product), C.c_int, C.POINTER(_i32)]),
     "jl_linear_fp8_floats": (_i64, [C.POINTER(Fp8Product)]),
     "jl_linear_fp8": (C.c_int, [C.POINTER(Fp8Product), _vp, C.c_int, _vp, _i64, C.c_int, _vp, _vp]),
     "jl_linear_gated_fp8": (C.c_int, [C.POINTER(Fp8Product), _i32, _f32, _f32, _f32, _vp, _i64, _vp, _i64, _vp]),
@@ -401,7 +402,7 @@ _LAYER_SIGNATURES = {
 LAYER_SYMBOLS = tuple(_LAYER_SIGNATURES)
 # which library a symbol lives in (jacobiforcing_amd/_build.py: LAYER_GROUPS); each carries its own jl_version / jl_last_error
 _SEQ_SYMBOLS = ("jl_retention", "jl_retention_pieces_ok", "jl_retention_pieces_run", "jl_retention_join", "jl_delta_rule", "jl_delta_chunks_ok", "jl_delta_chunks_floats", "jl_delta_chunks_run", "jl_linear_scan", "jl_linear_scan_chunked_ok", "jl_moe_route", "jl_moe_group", "jl_moe_tile_rows", "jl_moe_tile_pairs", "jl_moe_float_tiles", "jl_moe_router_blocks", "jl_moe_router_slices", "jl_moe_router_run", "jl_moe_few_ok", "jl_moe_few_run", "jl_moe_gemm", "jl_moe_gemm_gated")
-_FP8_SYMBOLS = ("jl_quantize_fp8", "jl_add_rmsnorm_fp8", "jl_gated_act_fp8", "jl_quantize_weight_fp8", "jl_linear_fp8_floats", "jl_linear_fp8", "jl_linear_gated_fp8")
+_FP8_SYMBOLS = ("jl_quantize_fp8", "jl_add_rmsnorm_fp8", "jl_gated_act_fp8", "jl_quantize_weight_fp8", "jl_fp8_cut", "jl_linear_fp8_floats", "jl_linear_fp8", "jl_linear_gated_fp8")
 _GROUP_OF = {**dict.fromkeys(_SEQ_SYMBOLS, "layers_seq"), **dict.fromkeys(_FP8_SYMBOLS, "layers_fp8")}      # the others are in "layers"
 
 

@@ -611,6 +611,13 @@ static Fp8Plan fp8_plan(const jl_fp8_product *p, bool gated) {
     }
     return best;
 }
+extern "C" const char *jl_fp8_cut(const jl_fp8_product *p, int gated, int32_t *shares) {
+    static const char *const names[] = {"16x64", "32x64", "64x64", "64x128", "128x128", "128x128 two", "128x256", "256x256", "16x128 many", "32x128 many", "64x128 many", "16x256", "32x256", "64x256", "rows"};
+    static_assert(sizeof names / sizeof names[0] == F8_FEW + 1, "a name for each");
+    const Fp8Plan plan = !p || p->N <= 0 || p->O <= 0 || p->K <= 0 ? Fp8Plan{F8_FEW, 1} : fp8_plan(p, gated != 0);
+    if (shares) *shares = plan.splits;
+    return names[plan.tile];
+}
 extern "C" int64_t jl_linear_fp8_floats(const jl_fp8_product *p) {
     if (!p || p->N <= 0 || p->O <= 0 || p->K <= 0) return 0;
     const Fp8Plan plan = fp8_plan(p, false);
