@@ -4,8 +4,8 @@
 #include "jl_fp8.h"
 
 // ---- rows of a matrix, or of a unit of two column ranges of it: a wavefront takes 512 columns of a row ---------------------------------------------------
-// Bound by memory: 8192 x 3584 of bfloat16 19.4 us (4.5 TB/s read and written; a large copy reaches 4.9), of floats 27.1 (5.4); units of 4096 x 4864 21.9 (4.5), of 8192 x 18944 143 (5.4).  The unit's sigmoid on
-// the hardware's exponential and reciprocal leaves as many values in 8 bits on the other side of a border as the library's functions do (60 million of gelu: 74 float scales, 137 plain torch; silu 90 / 90),
+// Bound by memory: 8192 x 3584 of bfloat16 18.2 us (4.8 TB/s read and written; a large copy reaches 4.9), of floats 26.0 (5.6), with float scales 19.3 and 27.5; units of 4096 x 4864 21.9 - 23 (4.3 - 4.5), of
+// 8192 x 18944 143 (5.4).  The unit's sigmoid on the hardware's exponential and reciprocal leaves as many values in 8 bits on the other side of a border as the library's functions do (60 million of gelu: 82 float scales, 137 plain torch; silu 90 / 90),
 // and those take 26.7 us.  Rows that start anywhere: 8192 x 3585 of bfloat16 22.4 (a value at a time 49).
 struct Q8Unit { int kind, g_col, u_col; float limit, alpha, shift; };      // u_col < 0: no linear branch
 
@@ -68,7 +68,7 @@ extern "C" int jl_gated_act_fp8(const void *z, int dtype, int64_t N, int64_t ld,
 }
 
 // ---- residual update, norm, 8 bits -----------------------------------------------------------------------------------------------------------------------
-// Bound by memory: 8192 x 3584 of a float stream 66.4 us (4.9 TB/s), of bfloat16 38.2 (5.4); 4096 x 8192 of floats 59 (6.3).  One row 3.8: two waits for memory and a workgroup's sum.
+// Bound by memory: 8192 x 3584 of a float stream 66.4 us (4.9 TB/s), of bfloat16 38.2 (5.4); 4096 x 8192 of floats 59 (6.3).  One row 3.8 (from memory 4.9): two waits for memory and a workgroup's sum.
 // NW wavefronts share a row, 512 columns at a time in turn; a thread keeps its 8 * NC values between the sum of squares and the quantisation, so a row is read once and written once.  NC = 0: rows too
 // wide for that are read again, from where the same thread has stored the update.
 struct Q8Norm { int64_t x_ld; const void *y; int y_dtype; int64_t y_ld; const void *w; int w_dtype; float eps; int64_t N; int W; };
@@ -191,6 +191,7 @@ extern "C" int jl_add_rmsnorm_fp8(void *x, int dtype, int64_t x_ld, const void *
 }
 
 // ---- weights: a scale for each block of 128 x 128, a workgroup's -----------------------------------------------------------------------------------------
+// Bound by memory: 37888 x 3584 of bfloat16 79 us (5.1 TB/s read and written), of floats 129 (5.3).
 template <typename T, bool E8>
 __global__ __launch_bounds__(256) void fp8_weight_kernel(const T *__restrict__ w, int64_t ld, int64_t O, int K, Q8Out out) {
     __shared__ uint32_t most[4];

@@ -186,10 +186,13 @@ __global__ __launch_bounds__(1024) void fp8_few_gated_kernel(Fp8Product a, int F
 // LDS, and eight columns of the result that follow one another (32 h + 8 q + 4 e + i: accumulators 2 h + e of lanes of quad q) are a lane's whole store; for that the rows of a wavefront are
 // permuted on their way into LDS.  Unit u of a row of LDS lies at u ^ (row / 2 % 8): the sixteen rows that are read at once meet different banks.
 // GATED: the lower accumulators are gates, the others the linear branches of the same results.
-// Tiles of 256 x 256, one workgroup per CU that takes tile after tile, the next one's first stage on its way while results are made: 8192 x 8192 by 8192 412 us (2670 TFLOP/s), gated 8192 x 3584 by
-// 2 x 18944 870 (2560; a workgroup for each tile 6 % more, a twentieth of it the units).  Tiles of 128 x 256: 2048 x 18944 by 3584 128 us (2170), of 128 x 128 512 rows by 3584 by 4608 21.6.
+// Tiles of 256 x 256, one workgroup per CU that takes tile after tile, the next one's first stage on its way while results are made: 8192 x 8192 by 8192 412 - 433 us (2540 - 2670 TFLOP/s), gated 8192 x 3584
+// by 2 x 18944 870 - 930 by box (2390 - 2560; a workgroup for each tile 6 % more, a twentieth of it the units).  Float scales: 485 and 1085 - 1100.  Tiles of 128 x 256: 2048 x 18944 by 3584 130 us (2140), of
+// 128 x 128 512 rows by 3584 by 4608 21.8.
 // What bounds it: the way into a CU, some 60 GB/s of stages from L2 whatever the tile (a quarter of the loads left out of 128 x 128 and 128 x 256: 20 % less time; nothing loaded at all in 256 x 256: 15 % less),
-// then LDS (two thirds of the time reads or loads of a stage go through it) and the matrix cores (70 %, with 256 x 256).
+// then the matrix cores (busy 67 % of the time in 8192 x 8192 by 8192, 60 % in the gated product, 47 % in 2048 x 18944 by 3584) and LDS (reads alone 27 %; what a stage's loads take is not counted there).
+// Tiles are whole ones: where they fill the card once and a bit, as 4096 rows of 3584 by 4608 do (288 of 256 x 256, so 576 of 128 x 256 in three rounds), half of the time is lost.
+// The gated tile of 256 x 256 needs more than its 256 registers: 13 vectors of offsets and constants, unused in the loop over the stages, are spilled and read back one by one in aim(), between tiles.
 //   Lines from beyond L2 are touched a stage earlier (AHEAD: 458 -> 436; smaller tiles, whose rings are longer, lose by it).
 //   The early barrier: 476 -> 459; no branch among the loads, so that they and the products stay in the order of the source: 459 -> 440; that order kept by force: 428 -> 418.
 //   No loads into registers in the loop: the compiler waits for those with everything on its way (529 -> 458, with results in stores of 16 bytes).

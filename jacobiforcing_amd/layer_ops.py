@@ -1210,7 +1210,7 @@ def gated_norm_linear(raw: torch.Tensor, gate: torch.Tensor, w_norm: torch.Tenso
 
 # ---- 8-bit rows --------------------------------------------------------------------------------------------------------------------------------------------
 # e4m3 values in rows padded with zeros to whole blocks of 128 columns, a scale for each row and block (activations) or each 128 x 128 (weights): powers of two (float8_e8m0fnu, what the matrix
-# instructions apply by themselves) or float32 (as checkpoints have them).  A block with an infinity or a NaN is all NaN.
+# instructions apply by themselves) or float32.  A block with an infinity or a NaN is all NaN.
 FP8_BLOCK, FP8_LARGEST = 128, 448.0
 _SCALES = {torch.float8_e8m0fnu: N.JL_SCALE_E8M0, torch.float32: N.JL_SCALE_F32}
 
@@ -1292,7 +1292,8 @@ def quantize_fp8(x: torch.Tensor, scale_dtype: torch.dtype = torch.float8_e8m0fn
 
 
 def add_rmsnorm_fp8(x: torch.Tensor, y: Optional[torch.Tensor], w: Optional[torch.Tensor], eps: float, scale_dtype: torch.dtype = torch.float8_e8m0fnu) -> Fp8Rows:
-    """x [N, W] += y in place, rounded to x's type (None: nothing is added); returns rms_norm(x) * w in 8 bits, float in between.  x, y and w each float or bfloat16, row strides free."""
+    """x [N, W] += y in place, rounded to x's type (None: nothing is added); returns rms_norm(x) * w in 8 bits, float in between.  x, y and w each float or bfloat16, row strides free; y may be x,
+    but must not overlap it otherwise."""
     native = _fp8_native("add_rmsnorm_fp8", x, y, w, eps, scale_dtype)
     if native is not NotImplemented:
         return Fp8Rows(*native)
@@ -1365,7 +1366,8 @@ def _fp8_operands(x: Fp8Rows, w: Fp8Weight, what: str) -> "N.Fp8Product":
 
 def linear_fp8(x: Fp8Rows, w: Fp8Weight, bias: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """x [N, K] times w [O, K] transposed (+ bias [O]): float sums of the values times their scales, rounded once to ``out_dtype`` (float or bfloat16; the bias of either).
-    The matrix instructions keep of each eight neighbouring products what lies within 2^-13 of the largest: float results are 5e-5 to 3e-4 off for random operands, below what bfloat16 shows.  Up to 2^21 rows."""
+    The matrix instructions keep of each eight neighbouring products what lies within 2^-13 of the largest: float results are 5e-5 to 3e-4 off for random operands, below what bfloat16 shows.  Up to 2^21 rows.
+    Float scales of x and w are multiplied first: their product is to lie within a float's range (2^-126 to 2^128)."""
     native = _fp8_native("linear_fp8", *x, *w, bias, out_dtype)
     if native is not NotImplemented:
         return native
@@ -1383,7 +1385,8 @@ def linear_fp8(x: Fp8Rows, w: Fp8Weight, bias: Optional[torch.Tensor] = None, ou
 
 def linear_gated_fp8(x: Fp8Rows, w_gu: Fp8Weight, kind: int, limit: float = 0.0, alpha: float = 1.0, shift: float = 0.0) -> Fp8Rows:
     """``gated_act_fp8`` of ``linear_fp8``'s float sums in the product's launch: w_gu's rows are F gates and behind them F linear branches, F whole blocks of 128 (``gated_act_fp8`` takes others).
-    The result's scales have the operands' type."""
+    The result's scales have the operands' type.  The sums are as exact as ``linear_fp8``'s: some 0.3 % of the values fall to the other side of a border, a step of 8 bits, against sums in 32 bits
+    (16- or 32-bit operands and ``gated_act_fp8`` where that matters)."""
     native = _fp8_native("linear_gated_fp8", *x, *w_gu, kind, limit, alpha, shift)
     if native is not NotImplemented:
         return Fp8Rows(*native)
@@ -1394,6 +1397,7 @@ def linear_gated_fp8(x: Fp8Rows, w_gu: Fp8Weight, kind: int, limit: float = 0.0,
         r = _fp8_rows(p.N, p.O // 2, x.scale.dtype, x.data.device)
         N.check_layers(N.layers().jl_linear_gated_fp8(p, int(kind), float(limit), float(alpha), float(shift), *_fp8_out(r)[:4], _stream(r.data.device)), "jl_linear_gated_fp8")
     return r
+
 
 def polynorm(z: torch.Tensor, coef: torch.Tensor, eps: float) -> torch.Tensor:
     """c0 n(z) + c1 n(z^2) + c2 n(z^3) + c3 with n(u) = u / rms(u) over a row; z [N, F], coef four floats."""
