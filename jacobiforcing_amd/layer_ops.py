@@ -1266,10 +1266,8 @@ _H8 = None                                           # the host side that the li
 
 
 def _fp8_native(name: str, *args):
-    """The call's native host side, or NotImplemented."""
+    """The call's native host side, or NotImplemented.  (A compiler does not follow it: the graph ends there, and the call runs as it is.)"""
     global _H8
-    if is_dynamo_compiling():
-        return NotImplemented
     h = _H or _host()
     if _H8 is not h:
         _H8 = N.host_fp8(h)
@@ -1371,15 +1369,16 @@ def linear_fp8(x: Fp8Rows, w: Fp8Weight, bias: Optional[torch.Tensor] = None, ou
     native = _fp8_native("linear_fp8", *x, *w, bias, out_dtype)
     if native is not NotImplemented:
         return native
-    p = _fp8_operands(x, w, "linear_fp8")
     _no_gradient("linear_fp8", *x, *w, bias)
+    p = _fp8_operands(x, w, "linear_fp8")
+    n, o = x.data.shape[0], w.data.shape[0]
     if bias is not None:
-        _need(bias.shape == (p.O,) and bias.is_contiguous() and bias.device == x.data.device, "linear_fp8: a bias has O entries")
+        _need(bias.shape == (o,) and bias.is_contiguous() and bias.device == x.data.device, "linear_fp8: a bias has O entries")
     codes = _code(bias.dtype) if bias is not None else N.JL_F32, _code(out_dtype)
     with torch.cuda.device(x.data.device):
-        out, floats = torch.empty((p.N, p.O), dtype=out_dtype, device=x.data.device), N.layers().jl_linear_fp8_floats(p)
+        out, floats = torch.empty((n, o), dtype=out_dtype, device=x.data.device), N.layers().jl_linear_fp8_floats(p)
         scratch = torch.empty(floats, dtype=torch.float32, device=out.device) if floats else None
-        N.check_layers(N.layers().jl_linear_fp8(p, _ptr(bias), codes[0], _ptr(out), p.O, codes[1], _ptr(scratch), _stream(out.device)), "jl_linear_fp8")
+        N.check_layers(N.layers().jl_linear_fp8(p, _ptr(bias), codes[0], _ptr(out), o, codes[1], _ptr(scratch), _stream(out.device)), "jl_linear_fp8")
     return out
 
 
@@ -1390,11 +1389,12 @@ def linear_gated_fp8(x: Fp8Rows, w_gu: Fp8Weight, kind: int, limit: float = 0.0,
     native = _fp8_native("linear_gated_fp8", *x, *w_gu, kind, limit, alpha, shift)
     if native is not NotImplemented:
         return Fp8Rows(*native)
-    p = _fp8_operands(x, w_gu, "linear_gated_fp8")
     _no_gradient("linear_gated_fp8", *x, *w_gu)
-    _need(p.O > 0 and p.O % (2 * FP8_BLOCK) == 0, "linear_gated_fp8: gates and linear branches in whole blocks of 128 rows")
+    p = _fp8_operands(x, w_gu, "linear_gated_fp8")
+    n, o = x.data.shape[0], w_gu.data.shape[0]
+    _need(o > 0 and o % (2 * FP8_BLOCK) == 0, "linear_gated_fp8: gates and linear branches in whole blocks of 128 rows")
     with torch.cuda.device(x.data.device):
-        r = _fp8_rows(p.N, p.O // 2, x.scale.dtype, x.data.device)
+        r = _fp8_rows(n, o // 2, x.scale.dtype, x.data.device)
         N.check_layers(N.layers().jl_linear_gated_fp8(p, int(kind), float(limit), float(alpha), float(shift), *_fp8_out(r)[:4], _stream(r.data.device)), "jl_linear_gated_fp8")
     return r
 
