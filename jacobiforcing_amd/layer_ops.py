@@ -1256,7 +1256,9 @@ def _row_stride(t: torch.Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
-def _no_gradient(what: str, *tensors: Optional[torch.Tensor]) -> None:
+def _launchable(what: str, *tensors: Optional[torch.Tensor]) -> None:
+    """Refuses what a launch would not do: be recorded in a trace, which would run again without it, or leave a gradient."""
+    _need(torch._C._get_tracing_state() is None and torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is None, f"{what} cannot be recorded in a trace (torch.compile runs it as it is)")
     dual = forward_ad._current_level >= 0
     _need(not any(t is not None and (t.requires_grad and torch.is_grad_enabled() or dual and forward_ad.unpack_dual(t).tangent is not None) for t in tensors),
           f"{what} has no gradient: call it where none is wanted")
@@ -1281,7 +1283,7 @@ def quantize_fp8(x: torch.Tensor, scale_dtype: torch.dtype = torch.float8_e8m0fn
     if native is not NotImplemented:
         return Fp8Rows(*native)
     _matrix(x, "quantize_fp8")
-    _no_gradient("quantize_fp8", x)
+    _launchable("quantize_fp8", x)
     code, (n, W) = _code(x.dtype), x.shape
     with torch.cuda.device(x.device):
         r = _fp8_rows(n, W, scale_dtype, x.device)
@@ -1296,7 +1298,7 @@ def add_rmsnorm_fp8(x: torch.Tensor, y: Optional[torch.Tensor], w: Optional[torc
     if native is not NotImplemented:
         return Fp8Rows(*native)
     _matrix(x, "add_rmsnorm_fp8")
-    _no_gradient("add_rmsnorm_fp8", x, y, w)
+    _launchable("add_rmsnorm_fp8", x, y, w)
     n, W = x.shape
     _need(y is None or not x.is_inference() or torch.is_inference_mode_enabled(), "add_rmsnorm_fp8: an inference tensor is changed in inference mode only")
     if y is not None:
@@ -1321,7 +1323,7 @@ def gated_act_fp8(z: torch.Tensor, g_col: int, u_col: int, F_: int, kind: int, l
     if native is not NotImplemented:
         return Fp8Rows(*native)
     _matrix(z, "gated_act_fp8")
-    _no_gradient("gated_act_fp8", z)
+    _launchable("gated_act_fp8", z)
     _need(F_ > 0 and 0 <= g_col and g_col + F_ <= z.shape[1] and u_col + F_ <= z.shape[1], "gated_act_fp8: z [N, ld] with both column ranges inside")
     code, n = _code(z.dtype), z.shape[0]
     with torch.cuda.device(z.device):
@@ -1334,7 +1336,7 @@ def gated_act_fp8(z: torch.Tensor, g_col: int, u_col: int, F_: int, kind: int, l
 def fp8_weight(w: torch.Tensor, scale_dtype: torch.dtype = torch.float8_e8m0fnu) -> Fp8Weight:
     """Weights w [O, K] (float or bfloat16) in 8 bits, a scale for each block of 128 x 128 (formed as ``quantize_fp8``'s)."""
     _matrix(w, "fp8_weight")
-    _no_gradient("fp8_weight", w)
+    _launchable("fp8_weight", w)
     _need(scale_dtype in _SCALES, f"fp8_weight: scales are float8_e8m0fnu or float32, got {scale_dtype}")
     code, (o, k) = _code(w.dtype), w.shape
     with torch.cuda.device(w.device):
@@ -1369,7 +1371,7 @@ def linear_fp8(x: Fp8Rows, w: Fp8Weight, bias: Optional[torch.Tensor] = None, ou
     native = _fp8_native("linear_fp8", *x, *w, bias, out_dtype)
     if native is not NotImplemented:
         return native
-    _no_gradient("linear_fp8", *x, *w, bias)
+    _launchable("linear_fp8", *x, *w, bias)
     p = _fp8_operands(x, w, "linear_fp8")
     n, o = x.data.shape[0], w.data.shape[0]
     if bias is not None:
@@ -1389,7 +1391,7 @@ def linear_gated_fp8(x: Fp8Rows, w_gu: Fp8Weight, kind: int, limit: float = 0.0,
     native = _fp8_native("linear_gated_fp8", *x, *w_gu, kind, limit, alpha, shift)
     if native is not NotImplemented:
         return Fp8Rows(*native)
-    _no_gradient("linear_gated_fp8", *x, *w_gu)
+    _launchable("linear_gated_fp8", *x, *w_gu)
     p = _fp8_operands(x, w_gu, "linear_gated_fp8")
     n, o = x.data.shape[0], w_gu.data.shape[0]
     _need(o > 0 and o % (2 * FP8_BLOCK) == 0, "linear_gated_fp8: gates and linear branches in whole blocks of 128 rows")

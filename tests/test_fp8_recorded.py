@@ -1,4 +1,4 @@
-"""8-bit operators under what looks on or compiles: torch.compile runs them as they are."""
+"""8-bit operators under what records calls or looks on: torch.compile runs them as they are; traces, which would be run again without the launches, are refused."""
 import pytest
 import torch
 
@@ -31,6 +31,27 @@ def test_compiled(native, monkeypatch):
         assert torch.equal(got, want)
         assert torch.equal(torch.compile(lambda w: LO.fp8_weight(w * 2).data.float(), backend="eager")(w), LO.fp8_weight(w * 2).data.float())
     torch._dynamo.reset()
+
+
+def calls(LO, x, w8):
+    x8 = LO.quantize_fp8(x)
+    return (lambda t: LO.quantize_fp8(t).data.float(), lambda t: LO.add_rmsnorm_fp8(t, None, None, 1e-6).data.float(), lambda t: LO.add_rmsnorm_fp8(x.clone(), t, None, 1e-6).data.float(),
+            lambda t: LO.add_rmsnorm_fp8(x.clone(), None, t[0], 1e-6).data.float(), lambda t: LO.gated_act_fp8(t, 0, 256, 256, 2).data.float(), lambda t: LO.fp8_weight(t).data.float(),
+            lambda t: LO.linear_fp8(x8, w8, t[0]))
+
+
+@gpu
+def test_traces():
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from jacobiforcing_amd import layer_ops as LO
+    x, _, w8 = inputs()
+    x8 = LO.quantize_fp8(x)
+    with torch.no_grad():
+        for call in (*calls(LO, x, w8), lambda t: LO.linear_fp8(x8, w8) + t[0], lambda t: LO.linear_gated_fp8(x8, w8, 2).data.float() + t[0, 0]):
+            with pytest.raises(ValueError, match="trace"):
+                torch.jit.trace(call, (x.clone(),), check_trace=False)
+            with pytest.raises(ValueError, match="trace"):
+                make_fx(call)(x.clone())
 
 
 @gpu
