@@ -1257,8 +1257,10 @@ def _row_stride(t: torch.Tensor) -> int:
 
 
 def _launchable(what: str, *tensors: Optional[torch.Tensor]) -> None:
-    """Refuses what a launch would not do: be recorded in a trace, which would run again without it, or leave a gradient."""
+    """Refuses what a launch on these tensors' memory would not do: be recorded in a trace, which would run again without it, read values that are not there as they stand (lazily negated views), or
+    leave a gradient."""
     _need(torch._C._get_tracing_state() is None and torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is None, f"{what} cannot be recorded in a trace (torch.compile runs it as it is)")
+    _need(not any(t is not None and (t.is_neg() or t._is_zerotensor()) for t in tensors), f"{what}: tensors whose memory holds their values (resolve_neg)")
     dual = forward_ad._current_level >= 0
     _need(not any(t is not None and (t.requires_grad and torch.is_grad_enabled() or dual and forward_ad.unpack_dual(t).tangent is not None) for t in tensors),
           f"{what} has no gradient: call it where none is wanted")

@@ -1,4 +1,4 @@
-"""8-bit operators under what records calls or looks on: torch.compile runs them as they are; traces, which would be run again without the launches, are refused."""
+"""8-bit operators under what records or transforms calls: torch.compile runs them as they are; traces, which would be run again without the launches, and values that memory does not hold are refused."""
 import pytest
 import torch
 
@@ -38,6 +38,26 @@ def calls(LO, x, w8):
     return (lambda t: LO.quantize_fp8(t).data.float(), lambda t: LO.add_rmsnorm_fp8(t, None, None, 1e-6).data.float(), lambda t: LO.add_rmsnorm_fp8(x.clone(), t, None, 1e-6).data.float(),
             lambda t: LO.add_rmsnorm_fp8(x.clone(), None, t[0], 1e-6).data.float(), lambda t: LO.gated_act_fp8(t, 0, 256, 256, 2).data.float(), lambda t: LO.fp8_weight(t).data.float(),
             lambda t: LO.linear_fp8(x8, w8, t[0]))
+
+
+@gpu
+@pytest.mark.parametrize("native", [True, False])
+def test_values_that_memory_does_not_hold(native, monkeypatch):
+    from jacobiforcing_amd import _native as N, layer_ops as LO
+    x, _, w8 = inputs()
+    if not native:
+        monkeypatch.setattr(LO, "_H", N._NoHost())
+    for call in calls(LO, x, w8):
+        lazy = torch._neg_view(x.clone())
+        with torch.no_grad():
+            with pytest.raises(ValueError, match="resolve_neg"):
+                call(lazy)
+            call(lazy.resolve_neg())
+    a = torch.complex(x, x).conj().imag                 # every other float, besides
+    with pytest.raises(ValueError):
+        LO.quantize_fp8(a)
+    with pytest.raises(ValueError, match="resolve_neg"):
+        LO.linear_fp8(LO.Fp8Rows(LO.quantize_fp8(x, F32).data, torch._neg_view(LO.quantize_fp8(x, F32).scale)), LO.fp8_weight(torch.ones(128, 512, device="cuda"), F32))
 
 
 @gpu
